@@ -182,7 +182,8 @@ __device__ __forceinline__ void plain_row(const PackedParams &p, const Block &b,
         dot += dpp_move<0x141>(dot);
         dot += dpp_move<0x140>(dot);
         const float m_new = fmaxf(m, dot);
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new), e = __builtin_amdgcn_exp2f(dot - m_new);
+        const float base = m_new == -INFINITY ? 0.f : m_new;     // seen scores of -inf alone so far: weights 0
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new), e = __builtin_amdgcn_exp2f(dot - base);
         l = l * alpha + e;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * alpha + e * (float)v[j * p.v_rs + i];
@@ -190,13 +191,13 @@ __device__ __forceinline__ void plain_row(const PackedParams &p, const Block &b,
     }
     float mt = fmaxf(m, __shfl_xor(m, 16, 64));
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);      // (weights 0 times what is not finite stay NaN)
     l *= f;
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        float a = l == 0.f || f == 0.f ? 0.f : acc[i] * f;
+        float a = acc[i] * f;
         a += __shfl_xor(a, 16, 64);
         a += __shfl_xor(a, 32, 64);
         if (g == 0) {

@@ -1,0 +1,64 @@
+"""Packed attention (include/cmhsa_packed.h) where single keys decide: infinite scores, marked keys at every boundary of tiles, chunks
+and pages' worth of keys, weights that round the same way.  Against the float64 oracle, in every kind of launch."""
+import numpy as np
+import pytest
+import torch
+
+import cmhsa
+from oracle import serving
+from test_packed_attention import TYPES, make, offsets, op
+
+EMPTY = [0] * 65                                                 # more sequences than a wave has lanes: tiles of 128 rows
+CODES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
+
+def cut_workspace(cu_q, cu_k, heads, kv_heads, d, dtype):
+    return cmhsa.load_library().cmhsa_packed_workspace_bytes(len(cu_q) - 1, int(cu_q[-1]), int(cu_k[-1]), heads, kv_heads, d, CODES[dtype])
+
+
+def run(dev, tensors, cu_q, cu_k, heads, kv_heads):
+    a, b = (torch.from_numpy(c).to(dev) for c in (cu_q, cu_k))
+    return op()(*(t.to(dev) for t in tensors), a, b, heads, kv_heads).double().cpu().numpy()
+
+
+# ---------------------------------------------------------------------------------------------------------- scores of -inf
+
+# (queries, keys) of the sequences; the launches are told apart by their sizes
+KINDS = {"short": ([12, 9], [12, 9]), "waves": ([70, 150], [70, 150]), "tiles": ([70, 150] + EMPTY, [70, 150] + EMPTY), "cut": ([5, 3], [1700, 1500])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 2, 64), (2, 1, 128)])
+@pytest.mark.parametrize("infinity", [-np.inf, np.inf])
+@pytest.mark.parametrize("kind,at", [(k, at) for k in ("short", "waves", "tiles") for at in (0, 1, 2, 3, 6)] + [("cut", at) for at in (0, 3, 128, 130, 1280, 1691)])
+def test_one_infinite_element_of_k_is_a_weight_of_zero(gpu_device, dtype, heads, kv_heads, d, infinity, kind, at):
+    """One element of K is infinite, and the queries' elements there have the sign that makes the score -inf: that key takes no
+    part, rows that see others are finite, and a row that sees nothing else is 0 / 0.  An infinite value at the first sequence's
+    last key sends the 16-bit types through the loop for what is not finite as well."""
+    rng = np.random.default_rng(at + d)
+    new, total = KINDS[kind]
+    cu_q, cu_k = offsets(new), offsets(total)
+    assert (cut_workspace(cu_q, cu_k, heads, kv_heads, d, dtype) > 0) == (kind == "cut")
+    tensors = make(rng, dtype, cu_q[-1], cu_k[-1], heads, kv_heads, d)
+    for h in range(heads):
+        tensors[0][:, h * d + 7] = -np.sign(infinity) * (tensors[0][:, h * d + 7].abs() + 0.25)
+    tensors[1][at, 7] = 0
+    tensors[2][total[0] - 1, 5] = np.inf
+    q, k, v = (t.double().numpy() for t in tensors)
+    reach = serving.packed_attention_f64(q, k, v, cu_q, cu_k, heads, kv_heads)[2]          # of the finite scores
+    tensors[1][at, 7] = infinity
+    k[at, 7] = infinity
+    with np.errstate(invalid="ignore"):
+        o, spread, _, weight = serving.packed_attention_f64(q, k, v, cu_q, cu_k, heads, kv_heads)
+    got = run(gpu_device, tensors, cu_q, cu_k, heads, kv_heads)
+    group, first = heads // kv_heads, total[0] - new[0]
+    hidden = np.zeros(o.shape, dtype=bool)                       # rows that see the infinite key and no other
+    if at == 0 and first == 0:
+        hidden[0, :group * d] = True
+    assert np.array_equal(np.isnan(o), hidden) and np.array_equal(np.isnan(got), hidden)
+    fine = np.isfinite(o)
+    assert (~fine & ~hidden).sum() == group and np.array_equal(got[~fine & ~hidden], o[~fine & ~hidden])
+    tol = serving.tolerance(dtype, (o, spread, reach, weight), max(total), d)
+    worst = np.abs(got[fine] - o[fine]) / tol[fine]
+    assert worst.max() <= 1.0, worst.max()
