@@ -62,3 +62,36 @@ def test_one_infinite_element_of_k_is_a_weight_of_zero(gpu_device, dtype, heads,
     tol = serving.tolerance(dtype, (o, spread, reach, weight), max(total), d)
     worst = np.abs(got[fine] - o[fine]) / tol[fine]
     assert worst.max() <= 1.0, worst.max()
+
+
+# ------------------------------------------------------------------------------------------------- weights of 16-bit types
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("kind,n", [("short", 31), ("waves", 900), ("tiles", 900), ("cut", 4000)])
+def test_equal_weights_that_round_the_same_way(gpu_device, dtype, kind, n):
+    """One key above n - 1 equal ones, whose weight lies just over half a step of the type above a representable one: rounded alike, all of them are off
+    the same way.  The last row's V is constant, and the quotient gives it back: numerator and denominator hold the same
+    weights, so only the fp32 sums (two steps a pair and add, 2^-22, over n / 2 in a row at most) and the output's rounding are left."""
+    h = {"bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    d = 64
+    new, total = ([3], [n]) if kind == "cut" else ([n], [n])
+    if kind == "tiles":
+        new, total = new + EMPTY, total + EMPTY
+    cu_q, cu_k = offsets(new), offsets(total)
+    assert (cut_workspace(cu_q, cu_k, 1, 1, d, dtype) > 0) == (kind == "cut")
+    # q = 8 (e_0 + .. + e_3), so that a score is the sum of four elements of K: 0 for the first key, ln(0.5 + 0.51 h) for the others, cut up over
+    # the four, since one of them would not hold it exactly enough
+    want = np.log(0.5 * (1 + 1.02 * h))
+    q, k, v = (torch.zeros((rows, d)) for rows in (int(cu_q[-1]), n, n))
+    q[:, :4] = 8
+    rest = want
+    for i in range(4):
+        part = torch.tensor(rest).to(TYPES[dtype])
+        k[1:, i] = part.float()
+        rest -= float(part)
+    assert abs(rest) < 1e-7
+    v[:] = 1.0 + 12 * 2 ** -7                                     # exact in both types
+    tensors = [t.to(TYPES[dtype]) for t in (q, k, v)]
+    got = run(gpu_device, tensors, cu_q, cu_k, 1, 1)
+    assert np.array_equal(got, np.full(got.shape, v[0, 0].item()))
