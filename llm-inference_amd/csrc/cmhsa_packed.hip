@@ -11,7 +11,7 @@
 // 8 (r / 4) + 4 (lane / 32) + r % 4, and V^T is read with its 16 keys in that order.  V stays as it comes (rows of keys) and
 // is transposed by the LDS read itself (ds_read_b64_tr_b16).
 // SOFTMAX in the log2 domain, one pass.  Weights are taken against the running maximum of EARLIER tiles; only when a lane's
-// sum over the tile leaves [0, 2^12] (always at a row's first tile) is the tile's maximum formed and what was
+// sum over the tile leaves [0, 2^12] (2^15 for fp16; always at a row's first tile) is the tile's maximum formed and what was
 // accumulated rescaled.  Sums and statistics are fp32; bf16 / fp16 weights are rounded once, to nearest, before the second
 // product (half a step of the type: what the output's own rounding costs), and summed as rounded: weights that are off the same
 // way are off in numerator and denominator alike (bf16, 32/8 heads of 128, 8192 tokens 571 -> 573 us, 32 heads of 64, 4 x 4096 339 -> 336).
@@ -43,8 +43,6 @@ typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kRows = 128;                       // packed rows of a workgroup: four waves of 32
-constexpr float kSumLimit = 4096.f;
-              // weights stay within fp16's range
 
 struct PackedParams {
     const void *q, *k, *v;
@@ -211,8 +209,13 @@ __device__ __forceinline__ void plain_row(const PackedParams &p, const Block &b,
 
 // ------------------------------------------------------------------------------------------------------ the tiled kernel
 // How a type is computed: its parts, the type of a part, the keys of a tile.
-template <typename T> struct Form { using Part = T; static constexpr int kParts = 1, kKeys = 64; };
-template <> struct Form<float> { using Part = bf16_t; static constexpr int kParts = 3, kKeys = 32; };
+// kLift: weights are taken against 2^-kLift of the maximum; kLimit: the sum over a lane's share of a tile beyond which the
+// maximum is formed anew (16 weights of 2^kLift do not pass it).  fp16 has no more than 24 bits below 1: lifted by 8 a weight keeps
+// all of its bits down to 2^-22 of the largest and vanishes at 2^-33, so that a long tail below one large weight stays; none
+// reaches fp16's 65504.
+template <typename T> struct Form { using Part = T; static constexpr int kParts = 1, kKeys = 64; static constexpr float kLift = 0.f, kLimit = 4096.f; };
+template <> struct Form<float> { using Part = bf16_t; static constexpr int kParts = 3, kKeys = 32; static constexpr float kLift = 0.f, kLimit = 4096.f; };
+template <> struct Form<f16_t> { using Part = f16_t; static constexpr int kParts = 1, kKeys = 64; static constexpr float kLift = 8.f, kLimit = 32768.f; };
 
 __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c, bf16_t) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -363,7 +366,7 @@ struct Rows {
     static constexpr int P = Form<T>::kParts, KT = Form<T>::kKeys, kPartBytes = KT * D * 2, kSteps = D / 16, kOut = D / 32;
     int query, head, last;                                       // this lane's row, and the last key that it sees
     int k_lane, v_lane;                                          // where the lane reads in a tile of K, of V
-    float m, l;                                                  // m: both halves of a row; l: this half's share
+    float m, l;                                                  // m: both halves of a row (the maximum less kLift); l: this half's share
     s16x8 q[kSteps][P];
     f32x16 acc[kOut];
 
@@ -455,12 +458,12 @@ struct Rows {
         settle(s, x, sum, scale);
     }
     __device__ __forceinline__ void settle(const f32x16 &s, s16x8 (&x)[2][P], float sum, float scale) {
-        if (__any(!(sum <= kSumLimit))) {                        // also a NaN, and a row's first keys (m = -inf): a new maximum
+        if (__any(!(sum <= Form<T>::kLimit))) {                  // also a NaN, and a row's first keys (m = -inf): a new maximum
             float top = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[r]);
             top = fmaxf(top, other_half(top));
-            const float m_new = fmaxf(m, top * scale);
+            const float m_new = fmaxf(m, top * scale - Form<T>::kLift);
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
 #pragma unroll
             for (int i = 0; i < kOut; ++i)

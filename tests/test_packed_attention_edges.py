@@ -95,3 +95,30 @@ def test_equal_weights_that_round_the_same_way(gpu_device, dtype, kind, n):
     tensors = [t.to(TYPES[dtype]) for t in (q, k, v)]
     got = run(gpu_device, tensors, cu_q, cu_k, 1, 1)
     assert np.array_equal(got, np.full(got.shape, v[0, 0].item()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("kind,n", [("short", 31), ("waves", 700), ("tiles", 700), ("cut", 4000)])
+def test_a_long_tail_below_one_large_weight(gpu_device, dtype, kind, n):
+    """The first key has weight 1 and a value of 0, every other one a weight between 2^-29 and 2^-26 and a value of about 1000: what comes
+    out is the tail alone.  fp16 numbers end at 2^-24.  Bound: as in serving.tolerance, but a weight is off by half a step of
+    fp16 (2h, with the sum) or by 2^-33 of the largest weight, which is 1, whichever is more."""
+    rng = np.random.default_rng(n)
+    d, u, h = 64, 2.0 ** -24, {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    new, total = ([3], [n]) if kind == "cut" else ([n], [n])
+    if kind == "tiles":
+        new, total = new + EMPTY, total + EMPTY
+    cu_q, cu_k = offsets(new), offsets(total)
+    assert (cut_workspace(cu_q, cu_k, 1, 1, d, dtype) > 0) == (kind == "cut")
+    q, k, v = (torch.zeros((rows, d)) for rows in (int(cu_q[-1]), n, n))
+    q[:, 0] = 8
+    k[1:, 0] = torch.from_numpy(rng.uniform(-29, -26, n - 1) * np.log(2)).float()
+    v[1:] = torch.from_numpy(rng.uniform(800, 1200, (n - 1, d))).float()
+    tensors = [t.to(TYPES[dtype]) for t in (q, k, v)]
+    o, spread, reach, weight = serving.packed_attention_f64(*(t.double().numpy() for t in tensors), cu_q, cu_k, 1, 1)
+    off = 2 * (d + 16) * u * reach + (160 + 2 * (n + 16)) * u + (0 if dtype == "float32" else 2 * h)
+    tol = off * spread + h * np.abs(o) + (2.0 ** -25 + 2.0 ** -33 * (weight + n * np.abs(o)) if dtype == "float16" else 1e-37)
+    assert (o[-1] > 3 * tol[-1]).all()                           # an answer without the tail is out of bounds
+    worst = np.abs(run(gpu_device, tensors, cu_q, cu_k, 1, 1) - o) / tol
+    assert worst.max() <= 1.0, worst.max()
