@@ -52,6 +52,7 @@ struct PackedParams {
     int num_seqs, total_q, total_k, num_kv_heads, group, zero_rest;
     float scale_log2;
     float *partial;                              // states of (block, chunk of its keys); null: a block has all its keys to itself
+    int *chunk;                                  // behind them: the chunks' length, for the join
     float one_per_target;                        // one over the tickets aimed at for each K/V head
     int min_chunk;                               // the shortest chunk, a multiple of both tile lengths
     int tickets;                                 // of a launch that cuts, for each K/V head
@@ -134,10 +135,12 @@ __device__ __forceinline__ Block block_of_many(const PackedParams &p, int t) {
 // one chunk lie side by side, so that they find its keys in the cache.
 struct Tickets {
     int length, chunks, upto;                                    // the last two: of this lane's sequence
-    __device__ __forceinline__ Tickets(const PackedParams &p, const Offsets &o) {
-        // (both launches form the same sum; its roundings are less than the 2^-13 added)
+    // (the sum's roundings are less than the 2^-13 added)
+    static __device__ __forceinline__ int length_of(const PackedParams &p, const Offsets &o) {
         const float each = fminf(wave_sum((float)o.blocks * (float)(o.k1 - o.k0)) * p.one_per_target * 1.0001f, 1.0e9f);
-        length = ((int)each + p.min_chunk) / p.min_chunk * p.min_chunk;
+        return ((int)each + p.min_chunk) / p.min_chunk * p.min_chunk;
+    }
+    __device__ __forceinline__ Tickets(const Offsets &o, int length) : length(length) {
         chunks = max(1, (o.k1 - o.k0 + length - 1) / length);
         upto = prefix_sum(o.blocks * chunks);
     }
@@ -644,7 +647,9 @@ __device__ __forceinline__ bool work_of(const PackedParams &p, Block &b, Span &x
     x.state = nullptr;
     if (kCut) {
         const Offsets o(p);
-        const Tickets y(p, o);
+        const Tickets y(o, Tickets::length_of(p, o));
+        // the join takes it from here: a float sum need not come out alike in two kernels
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.chunk = y.length;
         int chunk;
         if (!y.find(p, o, t, b, chunk)) return false;            // more workgroups than tickets
         x.from = chunk * y.length;
@@ -1003,13 +1008,13 @@ __global__ __launch_bounds__(kJoinThreads) void packed_join_kernel(PackedParams 
     if (p.zero_rest && part == 0 && threadIdx.x < 256) zero_rows<T, D>(p, t, kvh, __builtin_amdgcn_readfirstlane(places.q0), __builtin_amdgcn_readlane(places.q1, p.num_seqs - 1));
     const Block b = places.block(p, t);
     if (b.rows == 0) return;
-    const Tickets tickets(p, places);
+    const Tickets tickets(places, __builtin_amdgcn_readfirstlane(*p.chunk));
     const int blocks = __builtin_amdgcn_readlane(places.blocks, b.seq), first = tickets.first(places, b);
     const int r = part * kRowsHere + (int)threadIdx.x / kThreadsRow, d = (int)threadIdx.x % kThreadsRow * 4, row = b.first + r;
     if (row >= b.rows) return;
     const int query = row / p.group, head = kvh * p.group + row - query * p.group, last = b.nk - b.nq + query;
     const int count = last >= 0 ? last / tickets.length + 1 : 0;       // chunks that the row sees something of
-    if (first + (int64_t)(count - 1) * blocks >= p.tickets) return;      // (offsets that do not ascend: there is no such state)
+    if (first < 0 || first + (int64_t)(count - 1) * blocks >= p.tickets) return;     // (offsets that do not ascend: there is no such state)
     const int64_t step = (int64_t)blocks * p.num_kv_heads * state_floats(D);
     const float *state = p.partial + ((int64_t)first * p.num_kv_heads + kvh) * state_floats(D);
     // eight chunks' statistics and sums at once, past the last one its own again with factor 0
@@ -1091,6 +1096,7 @@ Plan plan_of(int num_seqs, int64_t total_q, int64_t total_k, int num_kv_heads, i
     plan.tickets = plan.split ? plan.target + plan.blocks + 1 : plan.blocks + 1;
     return plan;
 }
+size_t states_bytes(const Plan &plan, int num_kv_heads, int head_dim) { return (size_t)plan.tickets * num_kv_heads * state_floats(head_dim) * sizeof(float); }
 
 }  // namespace
 
@@ -1099,7 +1105,7 @@ extern "C" {
 size_t cmhsa_packed_workspace_bytes(int num_seqs, int total_q, int total_k, int num_heads, int num_kv_heads, int head_dim, int dtype) {
     if (num_seqs <= 0 || total_q <= 0 || total_k <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
     const Plan plan = plan_of(num_seqs, total_q, total_k, num_kv_heads, num_heads / num_kv_heads, dtype, head_dim);
-    return plan.split ? (size_t)plan.tickets * num_kv_heads * state_floats(head_dim) * sizeof(float) : 0;
+    return plan.split ? states_bytes(plan, num_kv_heads, head_dim) + 16 : 0;
 }
 
 int cmhsa_packed_fwd(const void *q, const void *k, const void *v, void *o,
@@ -1137,6 +1143,7 @@ int cmhsa_packed_fwd(const void *q, const void *k, const void *v, void *o,
     p.num_kv_heads = num_kv_heads; p.group = (int)group; p.zero_rest = zero_rest;
     p.scale_log2 = head_dim == 64 ? 0.18033688011112042f : 0.12751743082459868f;      // log2(e) / sqrt(head_dim)
     p.partial = plan.split ? static_cast<float *>(workspace) : nullptr;
+    p.chunk = plan.split ? reinterpret_cast<int *>(static_cast<char *>(workspace) + states_bytes(plan, num_kv_heads, head_dim)) : nullptr;
     p.one_per_target = 1.f / (float)plan.target;
     p.min_chunk = 128;                                           // (fp32, 4 x 16 tokens on 1000: 17.1 us, with 256 20.0)
     p.tickets = (int)plan.tickets;

@@ -122,3 +122,23 @@ def test_a_long_tail_below_one_large_weight(gpu_device, dtype, kind, n):
     assert (o[-1] > 3 * tol[-1]).all()                           # an answer without the tail is out of bounds
     worst = np.abs(run(gpu_device, tensors, cu_q, cu_k, 1, 1) - o) / tol
     assert worst.max() <= 1.0, worst.max()
+
+
+# ------------------------------------------------------------------------------------------------------------ cut launches
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,total", [([1], [1700]), ([3, 1], [1600, 5001]), ([300], [4096])], ids=str)
+def test_the_join_is_handed_the_chunk_length(gpu_device, new, total):
+    """It lies behind the states in the workspace: blocks times keys over the chunks aimed at (1024 of heads of 64), rounded up to 128."""
+    cu_q, cu_k = offsets(new), offsets(total)
+    heads, d = 2, 64
+    need = cut_workspace(cu_q, cu_k, heads, heads, d, "bfloat16")
+    tensors = [t.to(gpu_device) for t in make(np.random.default_rng(1), "bfloat16", cu_q[-1], cu_k[-1], heads, heads, d)]
+    space = torch.full((need,), 85, dtype=torch.uint8, device=gpu_device)
+    a, b = (torch.from_numpy(c).to(gpu_device) for c in (cu_q, cu_k))
+    got = cmhsa.attention_packed_fwd(*tensors, a, b, heads, heads, workspace=space)
+    each = sum(-(-n // 128) * t for n, t in zip(new, total)) / 512
+    assert space[need - 16:].view(torch.int32)[0].item() == int(each * 1.0001 + 128) // 128 * 128
+    assert torch.equal(got, op()(*tensors, a, b, heads, heads))
+
+
