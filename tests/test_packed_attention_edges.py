@@ -142,3 +142,66 @@ def test_the_join_is_handed_the_chunk_length(gpu_device, new, total):
     assert torch.equal(got, op()(*tensors, a, b, heads, heads))
 
 
+# ------------------------------------------------------------------------------------------------------ every key, once
+
+EVERY = {"short": [([20, 32, 7], [20, 32, 7])], "waves": [([230, 300], [230, 300]), ([9], [600]), ([65], [129])],
+         "tiles": [([230, 300] + EMPTY, [230, 300] + EMPTY), ([3, 1, 2] + EMPTY, [1000, 64, 65] + EMPTY), ([250] * 30, [257] * 30)],
+         "cut": [([1], [1700]), ([3, 1], [1600, 5001]), ([1, 2, 1, 1, 1], [31, 1, 9000, 256, 1153])]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,d", [(8, 4, 64), (4, 4, 128)])
+@pytest.mark.parametrize("kind,new,total", [(kind, *case) for kind in EVERY for case in EVERY[kind]], ids=str)
+def test_every_key_counts_once(gpu_device, dtype, heads, kv_heads, d, kind, new, total):
+    """q = 0: all weights are one number.  Each column of V holds 256 at one key and 0 elsewhere, a call after the other until every key has been
+    marked: a row's output is 256 over the keys that it sees, exactly but for the quotient's and the output's roundings (3 u and
+    h), or 0.  A key that is lost or taken twice changes one column by all of it."""
+    cu_q, cu_k = offsets(new), offsets(total)
+    assert (cut_workspace(cu_q, cu_k, heads, kv_heads, d, dtype) > 0) == (kind == "cut")
+    off = 3 * 2.0 ** -24 + {"float32": 0, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    columns, longest = kv_heads * d, max(total)
+    a, b = (torch.from_numpy(c).to(gpu_device) for c in (cu_q, cu_k))
+    q = torch.zeros((cu_q[-1], heads * d), dtype=TYPES[dtype], device=gpu_device)
+    k = torch.randn((cu_k[-1], columns), device=gpu_device).to(TYPES[dtype])
+    place = torch.cat([torch.arange(t) for t in total]).to(gpu_device)[:, None]            # of a key in its sequence
+    last = torch.cat([torch.arange(t - n, t) for n, t in zip(new, total)]).to(gpu_device)[:, None]     # key that a row sees
+    for at in range(0, longest, columns):
+        mark = at + torch.arange(columns, device=gpu_device)[None]
+        got = op()(q, k, (place == mark).to(TYPES[dtype]) * 256, a, b, heads, kv_heads).double()
+        mark = mark.view(kv_heads, 1, d).expand(kv_heads, heads // kv_heads, d).reshape(1, -1)
+        want = torch.where(mark <= last, 256 / (last + 1).double(), 0.0)
+        assert ((got - want).abs() <= off * want).all(), at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind,new,total", [(kind, *case) for kind in EVERY for case in EVERY[kind]], ids=str)
+def test_one_key_with_all_of_the_weight(gpu_device, dtype, d, kind, new, total):
+    """Each of four K/V heads has one key with a score of 64 where the others have 0, at every boundary of 32 keys in turn: rows that see it
+    return its value (the others weigh exp(-64) each: 2^-92), rows before it the mean of theirs."""
+    rng = np.random.default_rng(d)
+    heads = 4
+    cu_q, cu_k = offsets(new), offsets(total)
+    assert (cut_workspace(cu_q, cu_k, heads, heads, d, dtype) > 0) == (kind == "cut")
+    u, h = 2.0 ** -24, {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}[dtype]
+    a, b = (torch.from_numpy(c).to(gpu_device) for c in (cu_q, cu_k))
+    s = int(np.argmax(total))                                    # the longest sequence
+    n, t = new[s], total[s]
+    rows = slice(int(cu_q[s]), int(cu_q[s + 1]))
+    q = torch.zeros((cu_q[-1], heads, d), dtype=TYPES[dtype], device=gpu_device)
+    q[:, :, 3] = 8
+    v = torch.from_numpy(rng.uniform(1, 2, (cu_k[-1], heads, d)).astype(np.float32)).to(TYPES[dtype]).to(gpu_device)
+    marks = sorted({x for y in range(0, t + 1, 32) for x in (y - 1, y) if 0 <= x < t} | {t - 1})
+    for at in range(0, len(marks), heads):
+        key = torch.tensor([marks[min(at + i, len(marks) - 1)] for i in range(heads)], device=gpu_device)
+        k = torch.zeros((cu_k[-1], heads, d), dtype=TYPES[dtype], device=gpu_device)
+        k[int(cu_k[s]) + key, torch.arange(heads, device=gpu_device), 3] = 64 * d ** 0.5 / 8
+        got = op()(q.flatten(1), k.flatten(1), v.flatten(1), a, b, heads, heads).double().view(-1, heads, d)[rows]
+        mine = v[int(cu_k[s]):int(cu_k[s + 1])].double()
+        sums = mine.cumsum(0)[t - n:]
+        seen = torch.arange(t - n, t, device=gpu_device)[:, None, None]
+        want = torch.where(seen >= key[None, :, None], mine[key, torch.arange(heads, device=gpu_device)][None], sums / (seen + 1))
+        # (the mean's sums: a step of fp32 a key at most)
+        assert ((got - want).abs() <= (h + (t + 8) * u) * want + t * 2.0 ** -90).all(), marks[at]
