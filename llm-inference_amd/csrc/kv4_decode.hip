@@ -249,6 +249,7 @@ __global__ __launch_bounds__(W * 64, D == 128 && Parts<T>::n > 1 ? 3 : 4) void d
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
+    bool seen = false;                                           // uniform: a key counts, whatever its score
 
     const int stride = waves * kStep;
     int at = from + wave * kStep;
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(W * 64, D == 128 && Parts<T>::n > 1 ? 3 : 4) void d
         for (; at < to; at += stride) {
             bool masked = false;                                 // uniform: a subtile that ends past `to`, or has no page
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) masked |= x.first[u] > to - 16;
+            for (int u = 0; u < kSub; ++u) { masked |= x.first[u] > to - 16; seen |= x.first[u] < to; }
             // scores: rows of S^T are keys 4 quarter + r of each subtile
             float w[kSub][4];
 #pragma unroll
@@ -344,8 +345,10 @@ __global__ __launch_bounds__(W * 64, D == 128 && Parts<T>::n > 1 ? 3 : 4) void d
             __builtin_amdgcn_wave_barrier();
         }
     }
-    // the waves' states meet in LDS: O [col][D] in the wave's own area
+    // the waves' states meet in LDS: O [col][D] in the wave's own area.  A wave whose scores are all -inf has the lowest finite maximum: beside
+    // others it weighs nothing, and alone the result is 0 / 0; -inf is left for those that have no key.
     l = column_sum(l);
+    if (seen && m == -INFINITY) m = -3.4028234663852886e38f;
     __builtin_amdgcn_wave_barrier();
     float *state = reinterpret_cast<float *>(lds[wave]);
 #pragma unroll

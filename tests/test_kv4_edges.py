@@ -1,5 +1,5 @@
 """Single-token attention over the paged 4-bit cache (include/cmhsa_kv4.h) where single keys decide: every key marked in turn, one key with all of
-the weight at every boundary.  Expected values are a few operations in 64 bits over numbers that the cache holds exactly."""
+the weight at every boundary, scores of -inf.  Expected values are a few operations in 64 bits over numbers that the cache holds exactly."""
 import numpy as np
 import pytest
 import torch
@@ -69,3 +69,30 @@ def test_one_key_with_all_of_the_weight(gpu_device, dtype, d, page_size, lengths
         got = ops().kv4_decode(q.flatten(1), pages, table, ints(lengths, gpu_device), heads).double()[s].view(heads, d)
         want = v[first:first + t].double().view(t, heads, d)[key, torch.arange(heads, device=gpu_device)]
         assert ((got - want).abs() <= (HALF_STEP[dtype] + 4 * 2.0 ** -24) * want + 6 * t * 2.0 ** -89).all(), marks[at]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,d", [(2, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("lengths,width", [([100, 1, 33, 60], 128), ([3000, 400, 90, 2500], 3136)], ids=["one workgroup", "cut"])
+def test_scores_of_minus_infinity(gpu_device, dtype, heads, kv_heads, d, lengths, width):
+    """q . k passes fp32's range: the weight is 0 where another key's score is finite, and a sequence of nothing else is 0 / 0, as the formula
+    gives; where no position has a page the output is 0 all the same."""
+    page_size = 64
+    count = sum(-(-n // page_size) for n in lengths) + 2
+    pages, table = pool(count, kv_heads, page_size, d, gpu_device, fill=255), table_of(np.random.default_rng(3), lengths, page_size, count, gpu_device, width // page_size)
+    seq, place = places(lengths, gpu_device)
+    k, v = (torch.zeros((len(seq), kv_heads, d), device=gpu_device) for _ in range(2))
+    low = ((seq == 0) & (place < 70)) | (seq == 1) | ((seq == 2) & (place >= 1)) | (seq == 3)
+    k[low, :, 7] = -2.0 ** 120
+    v[~low] = 4
+    q = torch.zeros((4, heads, d), dtype=TYPES[dtype], device=gpu_device)
+    q[:, :, 7] = 2.0 ** 15
+    ops().kv4_append(k.flatten(1), v.flatten(1), pages, table, offsets(lengths, gpu_device), None)
+    got = ops().kv4_decode(q.flatten(1), pages, table, ints(lengths, gpu_device), heads)
+    assert (got[0] == 4).all() and (got[2] == 4).all()
+    assert torch.isnan(got[1]).all() and torch.isnan(got[3]).all()
+    table[3] = -1
+    table[1] = count
+    got = ops().kv4_decode(q.flatten(1), pages, table, ints(lengths, gpu_device), heads)
+    assert (got[0] == 4).all() and (got[2] == 4).all() and (got[1] == 0).all() and (got[3] == 0).all()
