@@ -1072,8 +1072,11 @@ void kernels_of(bool cut, bool waves, const void *&fwd, const void *&join) {
 //             bf16, 12 heads of 64: 512 tokens 14.0 / 8.0, 4 x 1 on 2000 14.0 / 19.6 (not), 25 heads, 8 x 16 on 1000 25.4 / 13.4
 //             fp16, 12 heads of 64: 2048 tokens 33.5 / 30.1, 4 x 800 22.1 / 24.8 (not), 25 heads, 8 x 1 on 1500 35.2 / 17.1; 16 heads of
 //             128, 512 tokens 19.8 / 12.5
-//           One sequence may have nearly all the keys: 16384 at most, 128 steps of a wave (fp32, 25 heads, 15 x 1 on 100 and one on 20000
-//             100, cut / 270; bf16 439, not cut / 160).
+//           One sequence may have nearly all the keys: beyond 16384 of them, 128 steps of a wave, a launch that meets the rule for
+//           cutting is cut; one that does not is better off here than in blocks, whatever the lengths.  In blocks / cut / so, 16 heads on 4:
+//             fp32, 64 x 1 on 1000 48.5 / 43.3 (cut) / 25.0; 25 heads, 15 x 1 on 100 and one on 20000 850 / 94 (cut) / 270
+//             bf16, 64 x 1 on 1000 25.7 / 22.2 / 14.4 (so); 25 heads, 15 x 1 on 100 and one on 20000 386 / 40 / 142 (so); 32/8 heads of 128,
+//             32 x 1 on 600 23.5 / 30.4 / 17.4 (so)
 //   split   otherwise, where all blocks of 128 rows are no more than a round of the chip (4 workgroups a CU for heads of 64, 2 for
 //           heads of 128, 1 for fp32 heads of 128) and the sequences' keys are long enough, on average, to pay for the states and
 //           the second launch: 1536 (fp32: 768), 768 where half of the CUs would have no workgroup.  Not cut / cut:
@@ -1087,10 +1090,11 @@ Plan plan_of(int num_seqs, int64_t total_q, int64_t total_k, int num_kv_heads, i
     const int64_t waves_blocks = total_q * group / 32 + num_seqs, places = waves_blocks * num_kv_heads, keys = num_seqs > 0 ? total_k / num_seqs : 0;
     const int64_t most = head_dim == 64 ? (keys >= 256 ? 1024 : 512) : dtype == CMHSA_F32 ? 640 : 384;
     const int64_t far = places >= (dtype == CMHSA_F32 ? 256 : 160) ? 2048 : dtype == CMHSA_F32 ? 768 : 1024;
-    plan.waves = num_seqs > 0 && num_seqs <= 64 && places <= most && keys > 32 && keys <= far && total_k <= 16384;
+    const bool few = num_seqs > 0 && num_seqs <= 64 && places <= most && keys > 32 && keys <= far;
     const int64_t round = head_dim == 64 ? 1024 : dtype == CMHSA_F32 ? 256 : 512;
     const int64_t least = dtype == CMHSA_F32 || plan.blocks * num_kv_heads <= 128 ? 768 : 1536;
-    plan.split = !plan.waves && num_seqs > 0 && num_seqs <= 64 && plan.blocks * num_kv_heads <= round && keys >= least;
+    plan.split = num_seqs > 0 && num_seqs <= 64 && plan.blocks * num_kv_heads <= round && keys >= least && (!few || total_k > 16384);
+    plan.waves = few && !plan.split;
     if (plan.waves) plan.blocks = waves_blocks;
     plan.target = (int)std::max<int64_t>(1, round / num_kv_heads);
     plan.tickets = plan.split ? plan.target + plan.blocks + 1 : plan.blocks + 1;

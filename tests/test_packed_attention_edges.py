@@ -205,3 +205,25 @@ def test_one_key_with_all_of_the_weight(gpu_device, dtype, d, kind, new, total):
         want = torch.where(seen >= key[None, :, None], mine[key, torch.arange(heads, device=gpu_device)][None], sums / (seen + 1))
         # (the mean's sums: a step of fp32 a key at most)
         assert ((got - want).abs() <= (h + (t + 8) * u) * want + t * 2.0 ** -90).all(), marks[at]
+
+
+# ------------------------------------------------------------------------------------------------------- skewed lengths
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,d,new,total", [(25, 25, 64, [1] * 16, [100] * 9 + [20000] + [100] * 6), (32, 8, 128, [1] * 32, [100] * 31 + [20000]), (16, 4, 64, [1] * 40, [500] * 40),
+                                                        (16, 4, 64, [3, 1, 40, 1], [100, 90, 50, 17000])], ids=["25x64", "32/8x128", "even", "four"])
+def test_one_long_sequence_among_short_ones(gpu_device, dtype, heads, kv_heads, d, new, total):
+    """More than 16384 keys in all, whose average says little: sampled rows and heads against the oracle, each with its own sequence's
+    length in the bound."""
+    cu_q, cu_k = offsets(new), offsets(total)
+    tensors = make(np.random.default_rng(7), dtype, cu_q[-1], cu_k[-1], heads, kv_heads, d)
+    got = run(gpu_device, tensors, cu_q, cu_k, heads, kv_heads)
+    q, k, v = (t.double().numpy() for t in tensors)
+    for s in sorted({0, 1, int(np.argmax(total)), len(total) - 1}):
+        for h in sorted({0, heads // 2, heads - 1}):
+            x, y = slice(h * d, (h + 1) * d), slice(h // (heads // kv_heads) * d, (h // (heads // kv_heads) + 1) * d)
+            rows, keys = slice(int(cu_q[s]), int(cu_q[s + 1])), slice(int(cu_k[s]), int(cu_k[s + 1]))
+            want = serving.attention_rows(q[rows, x], k[keys, y], v[keys, y], total[s] - new[s])
+            worst = np.abs(got[rows, x] - want[0]) / serving.tolerance(dtype, want, total[s], d)
+            assert worst.max() <= 1.0, (s, h, worst.max())
