@@ -783,8 +783,8 @@ def main() -> None:
     ap.add_argument("--fused-step-ops", action="store_true", help="embedding sum and next-token pick (arg-max, EOS, token write) as one HIP launch each (include/gpt2_step.h)")
     ap.add_argument("--fused-add-ln", action="store_true", help="every residual add + the LayerNorm after it as one HIP launch (include/gpt2_layernorm.h)")
     args = ap.parse_args()
-    if args.cache_bits == 4 and (not args.kv_cache or args.few_row_linear):
-        ap.error("--cache-bits 4 goes with --kv-cache, and not with --few-row-linear")
+    if args.cache_bits == 4 and (not args.kv_cache or args.few_row_linear or args.fused_step_ops):
+        ap.error("--cache-bits 4 goes with --kv-cache, and not with --few-row-linear or --fused-step-ops (one position for all rows)")
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))

@@ -1,0 +1,16 @@
+"""Command-line options of the generation harness that do not go together: refused before a model is built, not ignored."""
+import sys
+
+import pytest
+
+import gpt2_generation as gen
+
+
+@pytest.mark.parametrize("extra", [["--fused-step-ops"], ["--fused-add-ln", "--fused-step-ops"]], ids=" ".join)
+def test_step_ops_are_not_reported_where_they_are_not_used(monkeypatch, capsys, extra):
+    """gpt2_greedy_step takes one position for all rows; the paged loop has one for each."""
+    monkeypatch.setattr(gen, "build_model", lambda *a, **k: pytest.fail("a model was built"))
+    monkeypatch.setattr(sys, "argv", ["gpt2_generation.py", "--device", "cpu", "--kv-cache", "--cache-bits", "4", *extra])
+    with pytest.raises(SystemExit) as e:
+        gen.main()
+    assert e.value.code == 2 and "--fused-step-ops" in capsys.readouterr().err.splitlines()[-1]
