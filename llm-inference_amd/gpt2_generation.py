@@ -785,6 +785,8 @@ def main() -> None:
     args = ap.parse_args()
     if args.cache_bits == 4 and (not args.kv_cache or args.few_row_linear or args.fused_step_ops):
         ap.error("--cache-bits 4 goes with --kv-cache, and not with --few-row-linear or --fused-step-ops (one position for all rows)")
+    if args.cache_bits == 4 and args.backend != "CUSTOM_CUDA":
+        ap.error("--cache-bits 4 has its own HIP attention: no other --backend goes with it")
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
     rank = int(os.environ.get("RANK", "0"))

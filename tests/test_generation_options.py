@@ -14,3 +14,13 @@ def test_step_ops_are_not_reported_where_they_are_not_used(monkeypatch, capsys, 
     with pytest.raises(SystemExit) as e:
         gen.main()
     assert e.value.code == 2 and "--fused-step-ops" in capsys.readouterr().err.splitlines()[-1]
+
+
+@pytest.mark.parametrize("backend", ["NAIVE_PYTORCH", "PYTORCH_SDPA_MATH"])
+def test_no_other_attention_is_reported_than_the_one_that_runs(monkeypatch, capsys, backend):
+    """The paged loop has its own attention, whatever --backend says."""
+    monkeypatch.setattr(gen, "build_model", lambda *a, **k: pytest.fail("a model was built"))
+    monkeypatch.setattr(sys, "argv", ["gpt2_generation.py", "--device", "cpu", "--kv-cache", "--cache-bits", "4", "--backend", backend])
+    with pytest.raises(SystemExit) as e:
+        gen.main()
+    assert e.value.code == 2 and "--backend" in capsys.readouterr().err.splitlines()[-1]
