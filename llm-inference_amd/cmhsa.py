@@ -456,8 +456,10 @@ def kv4_block_bytes(page_size: int, head_dim: int) -> int:
     return page_size * head_dim // 16 * 17
 
 
-def _check_pages(pages: torch.Tensor, head_dim: int, page_table: torch.Tensor, num_seqs: int) -> int:
-    """The page size of a pool (num_pages, num_kv_heads, block bytes), checked against the table of `num_seqs` sequences."""
+def _check_pages(pages: torch.Tensor, head_dim: int, page_table: torch.Tensor, num_seqs: int, like: torch.Tensor) -> int:
+    """The page size of a pool (num_pages, num_kv_heads, block bytes) on like's device, checked against the table of `num_seqs` sequences."""
+    if pages.device != like.device:
+        raise ValueError("pages must be on the same device as the other tensors")
     if not pages.is_cuda or pages.dtype != torch.uint8 or pages.dim() != 3 or pages.stride(2) != 1 or (pages.shape[1] > 1 and pages.stride(1) != pages.shape[2]):
         raise ValueError("pages must be a (num_pages, num_kv_heads, block bytes) uint8 CUDA tensor with contiguous pages")
     page_size = pages.shape[2] * 16 // (17 * head_dim) if head_dim > 0 else 0
@@ -478,7 +480,7 @@ def kv4_append(K: torch.Tensor, V: torch.Tensor, pages: torch.Tensor, page_table
         raise ValueError("K and V must both be (rows, pages.shape[1] * head_dim)")
     _check_ints(cu_seqlens, "cu_seqlens", K)
     n, d = cu_seqlens.numel() - 1, K.shape[1] // pages.shape[1]
-    page_size = _check_pages(pages, d, page_table, n)
+    page_size = _check_pages(pages, d, page_table, n, K)
     if starts is not None:
         _check_ints(starts, "starts", K, n)
     with torch.cuda.device(K.device):
@@ -500,7 +502,7 @@ def kv4_gather(pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.
         raise ValueError("K and V must both be (rows, pages.shape[1] * head_dim)")
     _check_ints(cu_seqlens, "cu_seqlens", K)
     n = cu_seqlens.numel() - 1
-    page_size = _check_pages(pages, head_dim, page_table, n)
+    page_size = _check_pages(pages, head_dim, page_table, n, K)
     if starts is not None:
         _check_ints(starts, "starts", K, n)
     with torch.cuda.device(K.device):
@@ -521,7 +523,7 @@ def kv4_decode(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, l
     if num_heads <= 0 or q.shape[1] % num_heads or pages.dim() != 3 or pages.shape[1] < 1:
         raise ValueError("Feature dimension of q must be evenly divisible by the number of heads")
     n, d = q.shape[0], q.shape[1] // num_heads
-    page_size = _check_pages(pages, d, page_table, n)
+    page_size = _check_pages(pages, d, page_table, n, q)
     _check_ints(lengths, "lengths", q, n)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

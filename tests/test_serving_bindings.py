@@ -1,0 +1,37 @@
+"""What the ctypes forms of the serving calls (cmhsa.attention_packed_fwd, cmhsa.kv4_*) check before they call the library.  Tensors on devices that
+this machine need not have are stood in for: nothing here launches anything, but where marked."""
+import pytest
+import torch
+
+import cmhsa
+
+
+class On:
+    """A CPU tensor that says it lies on a device."""
+
+    def __init__(self, t, index):
+        self._t, self.device, self.is_cuda = t, torch.device("cuda", index), True
+
+    def __getattr__(self, name):
+        return getattr(self._t, name)
+
+
+@pytest.fixture
+def no_library(monkeypatch):
+    monkeypatch.setattr(cmhsa, "load_library", lambda: pytest.fail("the library was called"))
+
+
+@pytest.mark.parametrize("other", ["pages and table", "pages", "table", "offsets", "starts"])
+def test_a_pool_on_another_device_is_refused(no_library, other):
+    """A pool on another GPU is not this call's to read or write; the torch ops refuse it as well."""
+    at = lambda name: int(name in other)  # noqa: E731
+    x = On(torch.zeros(4, 128), 0)
+    pages, table = On(torch.zeros(3, 2, cmhsa.kv4_block_bytes(16, 64), dtype=torch.uint8), at("pages")), On(torch.zeros(1, 2, dtype=torch.int32), at("table"))
+    cu, starts, lengths = On(torch.tensor([0, 4], dtype=torch.int32), at("offsets")), On(torch.zeros(1, dtype=torch.int32), at("starts")), On(torch.zeros(1, dtype=torch.int32), at("offsets"))
+    with pytest.raises(ValueError, match="device"):
+        cmhsa.kv4_append(x, x, pages, table, cu, starts)
+    with pytest.raises(ValueError, match="device"):
+        cmhsa.kv4_gather(pages, table, cu, starts, 64, (x, x))
+    if other != "starts":
+        with pytest.raises(ValueError, match="device"):
+            cmhsa.kv4_decode(On(torch.zeros(1, 128), 0), pages, table, lengths, 2)
