@@ -554,6 +554,8 @@ def kv4_copy_pages(pages: torch.Tensor, src, dst) -> None:
         raise ValueError("src and dst must have the same number of pages")
     if pages.stride(-1) != 1 or (pages.shape[-2] > 1 and pages.stride(-2) != pages.shape[-1]):
         raise ValueError("a page's blocks must be contiguous")
+    if not all(0 <= page < pages.shape[-3] for page in (*src, *dst)):      # (a ctypes int keeps the low 32 bits of what it is given)
+        raise ValueError(f"src and dst must be page numbers below {pages.shape[-3]}")
     ints = ctypes.c_int * max(len(src), 1)
     with torch.cuda.device(pages.device):
         stream = torch.cuda.current_stream(pages.device).cuda_stream

@@ -35,3 +35,11 @@ def test_a_pool_on_another_device_is_refused(no_library, other):
     if other != "starts":
         with pytest.raises(ValueError, match="device"):
             cmhsa.kv4_decode(On(torch.zeros(1, 128), 0), pages, table, lengths, 2)
+
+
+@pytest.mark.parametrize("src,dst", [([1 << 32], [1]), ([0], [(1 << 32) + 1]), ([-(1 << 32)], [1]), ([3], [1]), ([0], [-1])], ids=str)
+@pytest.mark.parametrize("layers", [None, 2])
+def test_page_numbers_are_not_cut_to_32_bits(no_library, src, dst, layers):
+    shape = (3, 2, cmhsa.kv4_block_bytes(16, 64))
+    with pytest.raises(ValueError, match="page numbers"):
+        cmhsa.kv4_copy_pages(On(torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8), 0), src, dst)
