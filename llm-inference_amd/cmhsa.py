@@ -406,6 +406,15 @@ def _check_packed(t: torch.Tensor, name: str, like: torch.Tensor | None = None) 
         raise ValueError(f"{name} must be on the same device and of the same type as the other tensors")
 
 
+def _stride(t: torch.Tensor, dim: int, dense: int) -> int:
+    """t's stride over `dim`; `dense` where there is one row (page, layer) at most and its stride means nothing."""
+    return t.stride(dim) if t.shape[dim] > 1 else dense
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return _stride(t, 0, -(-t.shape[1] // 8) * 8)
+
+
 def _check_ints(t: torch.Tensor, name: str, like: torch.Tensor, count: int | None = None) -> None:
     if t.device != like.device or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1D int32 tensor on the same device")
@@ -442,7 +451,7 @@ def attention_packed_fwd(Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, cu_q
         raise ValueError("workspace must be a contiguous uint8 tensor on the same device")
     with torch.cuda.device(Q.device):
         stream = torch.cuda.current_stream(Q.device).cuda_stream
-        rc = load_library().cmhsa_packed_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), Q.stride(0), K.stride(0), V.stride(0), out.stride(0),
+        rc = load_library().cmhsa_packed_fwd(Q.data_ptr(), K.data_ptr(), V.data_ptr(), out.data_ptr(), _row_stride(Q), _row_stride(K), _row_stride(V), _row_stride(out),
                                              cu_q.data_ptr(), cu_k.data_ptr(), cu_q.numel() - 1, Q.shape[0], K.shape[0], num_heads, num_kv_heads, d,
                                              DTYPE_CODES[Q.dtype], 0 if given else 1, None if workspace is None else workspace.data_ptr(),
                                              0 if workspace is None else workspace.numel(), ctypes.c_void_p(stream))
@@ -485,7 +494,7 @@ def kv4_append(K: torch.Tensor, V: torch.Tensor, pages: torch.Tensor, page_table
         _check_ints(starts, "starts", K, n)
     with torch.cuda.device(K.device):
         stream = torch.cuda.current_stream(K.device).cuda_stream
-        rc = load_library().cmhsa_kv4_append(K.data_ptr(), V.data_ptr(), K.stride(0), V.stride(0), DTYPE_CODES[K.dtype], pages.data_ptr(), pages.stride(0), pages.shape[0],
+        rc = load_library().cmhsa_kv4_append(K.data_ptr(), V.data_ptr(), _row_stride(K), _row_stride(V), DTYPE_CODES[K.dtype], pages.data_ptr(), _stride(pages, 0, pages.shape[1] * pages.shape[2]), pages.shape[0],
                                              page_size, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_seqlens.data_ptr(),
                                              None if starts is None else starts.data_ptr(), n, K.shape[0], pages.shape[1], d, ctypes.c_void_p(stream))
     if rc != CMHSA_OK:
@@ -507,7 +516,7 @@ def kv4_gather(pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.
         _check_ints(starts, "starts", K, n)
     with torch.cuda.device(K.device):
         stream = torch.cuda.current_stream(K.device).cuda_stream
-        rc = load_library().cmhsa_kv4_gather(K.data_ptr(), V.data_ptr(), K.stride(0), V.stride(0), DTYPE_CODES[K.dtype], pages.data_ptr(), pages.stride(0), pages.shape[0],
+        rc = load_library().cmhsa_kv4_gather(K.data_ptr(), V.data_ptr(), _row_stride(K), _row_stride(V), DTYPE_CODES[K.dtype], pages.data_ptr(), _stride(pages, 0, pages.shape[1] * pages.shape[2]), pages.shape[0],
                                              page_size, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], cu_seqlens.data_ptr(),
                                              None if starts is None else starts.data_ptr(), n, K.shape[0], pages.shape[1], head_dim, 0, ctypes.c_void_p(stream))
     if rc != CMHSA_OK:
@@ -538,7 +547,7 @@ def kv4_decode(q: torch.Tensor, pages: torch.Tensor, page_table: torch.Tensor, l
         raise ValueError("workspace must be a contiguous uint8 tensor on the same device")
     with torch.cuda.device(q.device):
         stream = torch.cuda.current_stream(q.device).cuda_stream
-        rc = lib.cmhsa_kv4_decode(q.data_ptr(), out.data_ptr(), q.stride(0), out.stride(0), DTYPE_CODES[q.dtype], pages.data_ptr(), pages.stride(0), pages.shape[0],
+        rc = lib.cmhsa_kv4_decode(q.data_ptr(), out.data_ptr(), _row_stride(q), _row_stride(out), DTYPE_CODES[q.dtype], pages.data_ptr(), _stride(pages, 0, pages.shape[1] * pages.shape[2]), pages.shape[0],
                                   page_size, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lengths.data_ptr(), n, num_heads, pages.shape[1], d,
                                   workspace.data_ptr(), workspace.numel(), ctypes.c_void_p(stream))
     if rc != CMHSA_OK:
@@ -559,7 +568,7 @@ def kv4_copy_pages(pages: torch.Tensor, src, dst) -> None:
     ints = ctypes.c_int * max(len(src), 1)
     with torch.cuda.device(pages.device):
         stream = torch.cuda.current_stream(pages.device).cuda_stream
-        rc = load_library().cmhsa_kv4_copy_pages(pages.data_ptr(), pages.stride(0) if pages.dim() == 4 else 0, pages.shape[0] if pages.dim() == 4 else 1,
-                                                 pages.stride(-3), pages.shape[-3], pages.shape[-2] * pages.shape[-1], ints(*src), ints(*dst), len(src), ctypes.c_void_p(stream))
+        rc = load_library().cmhsa_kv4_copy_pages(pages.data_ptr(), _stride(pages, 0, 0) if pages.dim() == 4 else 0, pages.shape[0] if pages.dim() == 4 else 1,
+                                                 _stride(pages, -3, pages.shape[-2] * pages.shape[-1]), pages.shape[-3], pages.shape[-2] * pages.shape[-1], ints(*src), ints(*dst), len(src), ctypes.c_void_p(stream))
     if rc != CMHSA_OK:
         raise CmhsaError(rc, status_string(rc))

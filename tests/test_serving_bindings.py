@@ -43,3 +43,28 @@ def test_page_numbers_are_not_cut_to_32_bits(no_library, src, dst, layers):
     shape = (3, 2, cmhsa.kv4_block_bytes(16, 64))
     with pytest.raises(ValueError, match="page numbers"):
         cmhsa.kv4_copy_pages(On(torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8), 0), src, dst)
+
+
+@pytest.mark.gpu
+def test_a_single_row_has_no_stride(gpu_device):
+    """One row, page or layer cut out of something wider: its stride is not used, so it is not held to anything."""
+    d, block = 64, cmhsa.kv4_block_bytes(16, 64)
+    one = torch.randn(3, 2 * d + 1, device=gpu_device)[:1, :2 * d]
+    cu, n = torch.tensor([0, 1], dtype=torch.int32, device=gpu_device), torch.ones(1, dtype=torch.int32, device=gpu_device)
+    out = torch.zeros(3, 2 * d + 1, device=gpu_device)[:1, :2 * d]
+    # one key: its value, e V / e with e near 1: the part products left out are below 9 u of e V (u = 2^-24), sums, quotient and product 4 u
+    got = cmhsa.attention_packed_fwd(one, one, one, cu, cu, 2, 2, out=out).double()
+    assert ((got - one).abs() <= 13 * 2.0 ** -24 * one.abs()).all()
+    pages = torch.zeros(3, 2 * block + 1, dtype=torch.uint8, device=gpu_device)[:1, :2 * block].view(1, 2, block)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu_device)
+    row = torch.full((3, 2 * d + 1), 1.5, device=gpu_device)[:1, :2 * d]
+    cmhsa.kv4_append(row, row, pages, table, cu)
+    back = tuple(torch.zeros(3, 2 * d + 1, device=gpu_device)[:1, :2 * d] for _ in range(2))
+    cmhsa.kv4_gather(pages, table, cu, None, d, back)
+    assert torch.equal(back[0], row) and torch.equal(back[1], row)
+    got = cmhsa.kv4_decode(one, pages, table, n, 2, out=out).double()           # e 1.5 / e, e in three parts, no product left out: 4 u
+    assert ((got - 1.5).abs() <= 6 * 2.0 ** -24).all()
+    pool = torch.randint(0, 256, (2, 4 * 2 * block + 8), dtype=torch.uint8, device=gpu_device)[:1, :4 * 2 * block].view(1, 4, 2, block)
+    want = pool[0, 1].clone()
+    cmhsa.kv4_copy_pages(pool, [1], [3])
+    assert torch.equal(pool[0, 3], want)
