@@ -34,7 +34,8 @@ extern "C" {
 
 /* Requirements of all four calls: head_dim 64 or 128; page_size a power of two from 16 to 256; pages 16-B aligned,
  * page_stride (bytes) a multiple of 16 and at least num_kv_heads blocks; int32 arrays 4-B aligned.  Errors as in
- * include/cmhsa_packed.h. */
+ * include/cmhsa_packed.h; CMHSA_ERR_TOO_LARGE also for launches of 2^32 threads (append, gather: 32 a row and 512 elements of it; decode: 256 or 512
+ * a sequence, K/V head and 16 query heads). */
 
 /* Token r - cu_seqlens[s] of sequence s (row r of k and v: num_kv_heads * head_dim elements, row strides in elements,
  * multiples of 16 bytes) goes to position starts[s] + r - cu_seqlens[s] (starts NULL: 0).  Rows behind the last sequence

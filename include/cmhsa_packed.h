@@ -43,6 +43,7 @@ size_t cmhsa_packed_workspace_bytes(int num_seqs, int total_q, int total_k, int 
  * as they were.
  * Requirements: head_dim 64 or 128; num_heads a multiple of num_kv_heads; 16-B aligned pointers (cu: 4 B); row strides
  * multiples of 16 bytes and below 2^24 bytes.  total_q == 0 or num_seqs == 0 (without zero_rest) is a no-op.
+ * CMHSA_ERR_TOO_LARGE also where total_q * num_heads / 128 + num_seqs * num_kv_heads reaches 2^24 workgroups.
  * Returns CMHSA_OK, CMHSA_ERR_NULL_POINTER, CMHSA_ERR_BAD_SHAPE, CMHSA_ERR_HEAD_DIM, CMHSA_ERR_ALIGNMENT,
  * CMHSA_ERR_TOO_LARGE or a positive hipError_t. */
 int cmhsa_packed_fwd(const void *q, const void *k, const void *v, void *o,

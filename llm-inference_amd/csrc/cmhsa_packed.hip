@@ -1139,7 +1139,8 @@ int cmhsa_packed_fwd(const void *q, const void *k, const void *v, void *o,
         plan.tickets = plan.blocks + 1;
     }
     const int parts = kRows * head_dim / 4 / kJoinThreads;               // workgroups of a block in the join
-    if (plan.tickets * num_kv_heads > 0x7fffffff || (plan.blocks + 1) * num_kv_heads * parts > 0x7fffffff) return CMHSA_ERR_TOO_LARGE;
+    if (!fits_a_launch(plan.tickets * num_kv_heads, 256)) return CMHSA_ERR_TOO_LARGE;
+    if (plan.split && !fits_a_launch((plan.blocks + 1) * num_kv_heads * parts, kJoinThreads)) return CMHSA_ERR_TOO_LARGE;
     PackedParams p;
     p.q = q; p.k = k; p.v = v; p.o = o;
     p.q_rs = q_row_stride; p.k_rs = k_row_stride; p.v_rs = v_row_stride; p.o_rs = o_row_stride;

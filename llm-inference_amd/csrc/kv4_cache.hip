@@ -189,7 +189,7 @@ int rows_call(RowsParams p, bool append, int dtype, int64_t k_rs, int64_t v_rs, 
     const bool many = (int64_t)rows * 2 * p.chunks >= kManyWaves;
     const int each = many ? kWaveRows : 1;
     const int64_t waves = ((int64_t)rows + each - 1) / each * 2 * p.chunks;
-    if (waves > 0x7fffffffLL - 8) return CMHSA_ERR_TOO_LARGE;
+    if (!fits_a_launch((waves + 3) / 4, 256)) return CMHSA_ERR_TOO_LARGE;
     const void *fn = head_dim == 64 ? kernel_of<64>(append, dtype, many) : kernel_of<128>(append, dtype, many);
     void *args[] = {&p};
     const hipError_t e = hipLaunchKernel(fn, dim3((unsigned)((waves + 3) / 4)), dim3(256), args, 0, stream);
@@ -267,7 +267,7 @@ int cmhsa_kv4_copy_pages(uint8_t *pages, int64_t layer_stride, int layers, int64
     // pages that share bytes (an overlapping view) would be copied in no order
     if (layers > 1 && num_pages > 1 && layer_stride < (num_pages - 1) * page_stride + page_bytes && page_stride < (layers - 1) * layer_stride + page_bytes) return CMHSA_ERR_BAD_SHAPE;
     if (layers > 1 && layer_stride < page_bytes) return CMHSA_ERR_BAD_SHAPE;
-    if (layers > 65535 || page_bytes > (int64_t)1 << 40) return CMHSA_ERR_TOO_LARGE;
+    if (layers > 65535 || !fits_a_launch((page_bytes + kPieceBytes - 1) / kPieceBytes, 256)) return CMHSA_ERR_TOO_LARGE;
     // a page may be read often but written once, and never both: the pairs of a call have no order
     for (int i = 0; i < count; ++i)
         if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages) return CMHSA_ERR_BAD_SHAPE;

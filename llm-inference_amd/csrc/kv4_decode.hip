@@ -487,7 +487,7 @@ int cmhsa_kv4_decode(const void *q, void *o, int64_t q_row_stride, int64_t o_row
     if (plan.split && (!workspace || workspace_bytes < cmhsa_kv4_decode_workspace_bytes(num_seqs, table_width, page_size, num_heads, num_kv_heads, head_dim)))
         return CMHSA_ERR_WORKSPACE;
     const int64_t grid = plan.tickets * num_kv_heads * plan.head_chunks;
-    if (grid > 0x7fffffff || (int64_t)num_seqs * num_heads > 0x7fffffff) return CMHSA_ERR_TOO_LARGE;
+    if (!fits_a_launch(grid, plan.waves * 64) || (plan.split && !fits_a_launch((int64_t)num_seqs * num_heads, 256))) return CMHSA_ERR_TOO_LARGE;
     DecodeParams p;
     p.q = q; p.o = o; p.q_rs = q_row_stride; p.o_rs = o_row_stride;
     p.pool = kv4_pool(pages, page_stride, num_pages, page_size, page_table, table_stride, table_width);

@@ -12,6 +12,9 @@
 
 namespace serving {
 
+// A launch holds fewer than 2^32 threads: larger grids are refused here, so that no HIP error is left for the caller's next launch to find.
+inline bool fits_a_launch(int64_t workgroups, int threads) { return workgroups * threads <= 0xffffffffLL; }
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));

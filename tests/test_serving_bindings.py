@@ -1,5 +1,7 @@
 """What the ctypes forms of the serving calls (cmhsa.attention_packed_fwd, cmhsa.kv4_*) check before they call the library.  Tensors on devices that
 this machine need not have are stood in for: nothing here launches anything, but where marked."""
+import ctypes
+
 import pytest
 import torch
 
@@ -43,6 +45,20 @@ def test_page_numbers_are_not_cut_to_32_bits(no_library, src, dst, layers):
     shape = (3, 2, cmhsa.kv4_block_bytes(16, 64))
     with pytest.raises(ValueError, match="page numbers"):
         cmhsa.kv4_copy_pages(On(torch.zeros(shape if layers is None else (layers, *shape), dtype=torch.uint8), 0), src, dst)
+
+
+def test_launches_of_too_many_threads_are_refused():
+    """2^32 threads: an error of the launch itself would be left for the caller's next one to find.  (Nothing is read: the library
+    refuses before it launches.)"""
+    lib, at, block = cmhsa.load_library(), ctypes.c_void_p(0x1000), cmhsa.kv4_block_bytes(64, 64)
+    packed = lambda seqs, rows, heads, dtype=1: lib.cmhsa_packed_fwd(at, at, at, at, *[heads * 64] * 4, at, at, seqs, rows, rows, heads, heads, 64, dtype, 1, None, 0, None)  # noqa: E731
+    assert packed(1 << 22, 1 << 22, 4) == packed(1 << 24, 8, 1) == packed(1, 1 << 30, 2) == cmhsa.CMHSA_ERR_TOO_LARGE
+    pool = (at, 2 * block, 4, 64, at, 1, 1)
+    for rows_call, rest in ((lib.cmhsa_kv4_append, ()), (lib.cmhsa_kv4_gather, (1,))):
+        for rows in (1 << 27, (1 << 31) - 1025):
+            assert rows_call(at, at, 128, 128, 1, *pool, at, None, 1, rows, 2, 64, *rest, None) == cmhsa.CMHSA_ERR_TOO_LARGE
+    assert lib.cmhsa_kv4_decode(at, at, 256, 256, 1, *pool, at, 1 << 23, 4, 2, 64, None, 0, None) == cmhsa.CMHSA_ERR_TOO_LARGE
+    assert lib.cmhsa_kv4_copy_pages(at, 0, 1, 1 << 39, 2, 1 << 38, (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(1), 1, None) == cmhsa.CMHSA_ERR_TOO_LARGE
 
 
 @pytest.mark.gpu
