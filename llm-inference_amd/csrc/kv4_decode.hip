@@ -435,8 +435,11 @@ void kernels_of(int waves, const void *&decode, const void *&join) {
 
 // How a launch is laid out, by sizes that the host knows (the lengths themselves it does not).  Measured, in us a call:
 //   split      beyond 1024 positions where the workgroups would be few (12 of 2000 positions: 9.4 cut and joined, 12.4 not;
-//              96 of 1200: 10.9 and 9.8), beyond 2048 always (1600, one sequence of 4096 among 63 of 500: 28 and 34; all of
-//              4096: 115 and 109)
+//              96 of 1200: 10.9 and 9.8), beyond 2048 (1600, one sequence of 4096 among 63 of 500: 28 and 34; all of
+//              4096: 115 and 109) unless sequences are so many that every workgroup's look through their lengths costs more
+//              than one long sequence alone would: workgroups times sequences against 256 times the capacity.  Not cut / cut,
+//              all of 1000 and one as long as the table: 1024 x 8 K/V heads of 128, table of 16384 (512 times) 213 / 318, 303 / 388;
+//              of 131072 (64 times) 205 / 322, 1147 / 417; 256 x 8, of 16384 (32) 51 / 69, 158 / 89; 4096 x 1 of 64, of 4096 (4096) 53 / 180, 67 / 184
 //   per_head   chunks aimed at: one round of the chip, 3 workgroups a CU for heads of 128 (two of 131000, fp16: 65.4, and
 //              73.5 with 4 a CU, of which the last would wait), 4 for heads of 64
 //   waves      8 where few workgroups hold a sequence each (256 of 1000: 11.2, and 12.3 with 4), else 4
@@ -447,7 +450,7 @@ Plan plan_of(int num_seqs, int64_t capacity, int num_heads, int num_kv_heads, in
     Plan plan;
     plan.head_chunks = (num_heads / num_kv_heads + kCols - 1) / kCols;
     const int64_t each = (int64_t)num_kv_heads * plan.head_chunks, all = each * num_seqs, round = head_dim == 128 ? 768 : 1024;
-    plan.split = (capacity > 2048 || (capacity > 1024 && all < 64)) && num_seqs <= 65536;
+    plan.split = (capacity > 2048 || (capacity > 1024 && all < 64)) && num_seqs <= 65536 && all * num_seqs <= 256 * capacity;
     plan.per_head = (int)(each >= round ? 1 : round / each);
     plan.waves = plan.split || all >= 512 ? 4 : 8;
     plan.wave_keys = all >= 1024 ? 64 : 32;

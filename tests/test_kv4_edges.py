@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+import cmhsa
 from test_kv4_cache import TYPES, ints, offsets, ops, pool, table_of
 
 HALF_STEP = {"float32": 0.0, "bfloat16": 2.0 ** -8, "float16": 2.0 ** -11}      # of a rounded output (fp32: counted with the sums)
@@ -96,3 +97,14 @@ def test_scores_of_minus_infinity(gpu_device, dtype, heads, kv_heads, d, lengths
     table[1] = count
     got = ops().kv4_decode(q.flatten(1), pages, table, ints(lengths, gpu_device), heads)
     assert (got[0] == 4).all() and (got[2] == 4).all() and (got[1] == 0).all() and (got[3] == 0).all()
+
+
+@pytest.mark.gpu
+def test_many_sequences_in_a_long_table(gpu_device):
+    """More sequences than a look through all of their lengths pays for: not cut, and every key counts once all the same."""
+    rng = np.random.default_rng(4)
+    heads, kv_heads, d, page_size, width = 4, 2, 64, 64, 2112
+    lengths = [int(x) for x in rng.integers(0, 300, 599)] + [2100]
+    assert cmhsa.load_library().cmhsa_kv4_decode_workspace_bytes(600, width // page_size, page_size, heads, kv_heads, d) == 0
+    assert cmhsa.load_library().cmhsa_kv4_decode_workspace_bytes(64, width // page_size, page_size, heads, kv_heads, d) > 0
+    test_every_key_counts_once(gpu_device, "bfloat16", heads, kv_heads, d, page_size, lengths, width)
