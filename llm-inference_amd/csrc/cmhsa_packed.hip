@@ -24,7 +24,7 @@
 // BOUND.  Long sequences: by matrix instructions and the softmax's vector instructions, which the order given in step() lays
 // side by side.  Short ones: by a chain of dependent loads (offsets, then keys and queries) and by places for workgroups.
 // MEASURED, us (TFLOP/s of the pairs that are seen): bf16, 32/8 heads of 128: 16384 tokens 2218 (991), 4 x 4096 619 (888); 32 heads of
-// 64, 4 x 4096 360 (764).  fp32, 16 heads of 64, 8 x 4096 1445 (190), 32/8 of 128, 4096 tokens 760 (181): six times that is
+// 64, 4 x 4096 336 (818).  fp32, 16 heads of 64, 8 x 4096 1445 (190), 32/8 of 128, 4096 tokens 760 (181): six times that is
 // 1090 of the 1233 that a large bf16 library product reaches.  fp32, 25 heads of 64, 64 prompts of 1..512 tokens 58.8; fp16, 16/4
 // heads of 64, 16 x 100 tokens on 4000 61 (423); fp32, 12 heads, 8 tokens 5.1, 300 tokens 11.1.
 
@@ -1004,11 +1004,12 @@ __global__ __launch_bounds__(kJoinThreads) void packed_join_kernel(PackedParams 
     constexpr int kThreadsRow = D / 4, kRowsHere = kJoinThreads / kThreadsRow, kParts = kRows / kRowsHere;
     const int part = blockIdx.x % kParts, rest = blockIdx.x / kParts;
     const int kvh = rest % p.num_kv_heads, t = rest / p.num_kv_heads;
+    const int length = *p.chunk;                                 // asked for with the offsets, not behind them
     const Offsets places(p);
     if (p.zero_rest && part == 0 && threadIdx.x < 256) zero_rows<T, D>(p, t, kvh, __builtin_amdgcn_readfirstlane(places.q0), __builtin_amdgcn_readlane(places.q1, p.num_seqs - 1));
     const Block b = places.block(p, t);
     if (b.rows == 0) return;
-    const Tickets tickets(places, __builtin_amdgcn_readfirstlane(*p.chunk));
+    const Tickets tickets(places, __builtin_amdgcn_readfirstlane(length));
     const int blocks = __builtin_amdgcn_readlane(places.blocks, b.seq), first = tickets.first(places, b);
     const int r = part * kRowsHere + (int)threadIdx.x / kThreadsRow, d = (int)threadIdx.x % kThreadsRow * 4, row = b.first + r;
     if (row >= b.rows) return;
