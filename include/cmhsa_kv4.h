@@ -57,6 +57,7 @@ int cmhsa_kv4_gather(void *k, void *v, int64_t k_row_stride, int64_t v_row_strid
  *     o[s, h] = sum_j softmax_j( q[s, h] . K[j, g] / sqrt(head_dim) ) V[j, g]          g = h / (num_heads / num_kv_heads)
  * q, o: num_seqs rows of num_heads * head_dim elements of `dtype`, sharing no memory.  lengths: int32 in DEVICE memory, so that a captured
  * graph serves every step.  lengths[s] == 0, or outside [0, table_width * page_size]: nothing is read and o[s] = 0.
+ * Scores of -inf (q . K beyond fp32's range) weigh 0; a sequence that has no other is not a number.
  * workspace: device memory of at least cmhsa_kv4_decode_workspace_bytes(..) bytes, 16-B aligned, contents irrelevant
  * before and after (NULL where that is 0); calls that overlap in time must not share one. */
 size_t cmhsa_kv4_decode_workspace_bytes(int num_seqs, int table_width, int page_size, int num_heads, int num_kv_heads, int head_dim);

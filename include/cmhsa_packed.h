@@ -38,7 +38,10 @@ size_t cmhsa_packed_workspace_bytes(int num_seqs, int total_q, int total_k, int 
  * DEVICE memory, cu[0] = 0 for packing without a gap; cu_k may be cu_q.  o shares no memory with q, k or v.  A value outside [0, total] is taken as the
  * nearest one inside, and what ends before it starts is empty: no value reads or writes out of range, but which rows are
  * written where they do not ascend is not said.
- * dtype: CMHSA_F32 / CMHSA_BF16 / CMHSA_F16 for all four.  Statistics and sums are fp32 for every type.
+ * dtype: CMHSA_F32 / CMHSA_BF16 / CMHSA_F16 for all four.  Statistics and sums are fp32 for every type; a key's weight is its exponential
+ * against a running maximum, up to 2^15, so that values of v beyond about 2^112 over the number of keys may overflow in the sums.
+ * Up to 64 sequences a call get the faster layouts: short ones a wave each, the longest work first, keys cut between
+ * workgroups.  Beyond, every (sequence, K/V head, 128 rows) is a workgroup of its own, whatever its length.
  * zero_rest != 0 writes zeros to the rows of o that belong to no sequence (those from cu_q[num_seqs] on); 0 leaves them
  * as they were.
  * Requirements: head_dim 64 or 128; num_heads a multiple of num_kv_heads; 16-B aligned pointers (cu: 4 B); row strides
