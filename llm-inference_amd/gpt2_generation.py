@@ -581,7 +581,7 @@ class PagedGreedyGenerator:
             raise ValueError("max_tokens exceeds the model's context length")
         self.use_graphs, self.check_every, self.share_prefix, self.progress = use_graphs, check_every, share_prefix, progress
         heads = model.cfg["n_heads"]
-        self.cache = Kv4Cache(len(model.blocks), heads, model.cfg["emb_dim"] // heads, num_pages or batch * -(-max_tokens // page_size), batch,
+        self.cache = Kv4Cache(len(model.blocks), heads, model.cfg["emb_dim"] // heads, batch * -(-max_tokens // page_size) if num_pages is None else num_pages, batch,
                               max_tokens, page_size, self.device, ops)
         dev = self.device
         self.tokens = torch.zeros((batch, max_tokens + 1), dtype=torch.long, device=dev)    # +1: where a finished row's step would write

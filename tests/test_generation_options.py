@@ -24,3 +24,13 @@ def test_no_other_attention_is_reported_than_the_one_that_runs(monkeypatch, caps
     with pytest.raises(SystemExit) as e:
         gen.main()
     assert e.value.code == 2 and "--backend" in capsys.readouterr().err.splitlines()[-1]
+
+
+def test_a_pool_of_no_pages_is_refused():
+    """num_pages=0 is a number of pages, and too few; None is the default."""
+    from causal_self_attention import ScaledDotProductAttentionBackend as Backend
+
+    m = gen.build_model("gpt2", Backend.NAIVE_PYTORCH, "cpu", overrides=dict(emb_dim=64, n_heads=1, n_layers=1, vocab_size=11, context_length=32))
+    with pytest.raises(ValueError, match="num_pages"):
+        gen.PagedGreedyGenerator(m, 1, 32, use_graphs=False, page_size=16, num_pages=0, ops=object())
+    assert gen.PagedGreedyGenerator(m, 3, 20, use_graphs=False, page_size=16, ops=object()).cache.num_pages == 6
